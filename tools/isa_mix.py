@@ -39,7 +39,7 @@ def classify(op):
         return 'lds'
     if op in ('s_waitcnt', 's_nop'):
         return 'wait'
-    if op.startswith('s_load') or op.startswith('s_store') or op.startswith('s_buffer') or op in ('s_memtime', 's_memrealtime'):
+    if op.startswith('s_load') or op.startswith('s_buffer') or op in ('s_memtime', 's_memrealtime'):
         return 'smem'
     if op.startswith('s_'):
         return 'salu'
